@@ -14,7 +14,6 @@ Formats, shared by all three:
 * JumpReLU checkpoints: with u = pre - theta, a byte holds ceil(126 u / eps) inside the band
   |u| < eps, 127 above it and -128 below it; inside the band it stands for the middle of its step.
 """
-import functools
 import math
 import pathlib
 import sys
@@ -27,7 +26,6 @@ GROUP8 = 32          # columns that share a step in an 8-bit checkpoint
 BAND_STEPS = 126     # steps of a JumpReLU checkpoint in half a band
 
 
-@functools.cache
 def _package():
     root = str(pathlib.Path(__file__).resolve().parents[1] / "event-aware-sae-trainer_b200")
     if root not in sys.path:
