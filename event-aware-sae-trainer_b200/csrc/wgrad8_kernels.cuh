@@ -425,7 +425,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WgConfig<EXPAND, PAR
           code[q] = *reinterpret_cast<const uint4*>(raw + row * 128 + 16 * j);
           step2[q] = raw[WG_RAW_CODES + row * 16 + sb] * 0x00800080u;
         }
-        __syncwarp();   // the codes are in registers: their buffer may be filled again
+        // The reads above have to be over before TMA fills the buffer again. Nothing has
+        // used their values yet, and behind the epilogue's stores they can wait longer
+        // than the next copy takes; the fence orders them before it. 4096 tokens x 8192
+        // columns take 78 us with it for 1024 bf16 gradients, 67 for 256 of fp32 (77 and
+        // 67 without, when the codes of six stages later could be read).
+        fence_proxy_async_smem();
+        __syncwarp();
         if (lane == 0) mbar_arrive(&raw_empty[rst.s]);
         if (!wg_wait(&empty[st.s], st.ph ^ 1, abort_flag)) {
           ok = false;

@@ -140,6 +140,34 @@ def test_weight_grad(T, D, N, gdtype, transposed):
     assert (np.abs(off - want) <= room).all()
 
 
+@pytest.mark.parametrize("T,D,N,gdtype", [(4096, 8192, 1024, torch.bfloat16),
+                                         (2048, 20000, 512, torch.bfloat16),
+                                         (1000, 49152, 264, torch.bfloat16),
+                                         (4096, 16384, 512, torch.float32),
+                                         (1000, 1536, 16384, torch.float32)])
+@pytest.mark.parametrize("transposed", [False, True])
+def test_weight_grad_of_more_tiles_than_pairs_of_sms(T, D, N, gdtype, transposed):
+    """A pair of SMs goes on to a second tile while the first is still being stored
+    (slowest when transposed): every call gives the same bits, within the bound."""
+    B = _pkg()
+    gen = torch.Generator(device=DEV).manual_seed(T + D + N)
+    x = torch.randn(T, D, device=DEV, generator=gen).bfloat16()
+    g = (torch.randn(T, N, device=DEV, generator=gen) * 1e-3).to(gdtype)
+    a = B.checkpoint8(x)
+    v, g64 = a.dequantize(torch.float32).double(), g.double()
+    want, bound = g64.t() @ v, 2.0 ** -23 * (64 + T / 256) * (g64.abs().t() @ v.abs()) + 1e-37
+    del v, g64
+    other = torch.empty(256 << 20, device=DEV, dtype=torch.uint8)
+    first = None
+    for _ in range(5):
+        other.zero_()                    # the operands leave the L2 cache
+        got = a.weight_grad(g, transposed=transposed)
+        first = got if first is None else first
+        assert torch.equal(got, first)
+    got = first.t() if transposed else first
+    assert bool(((got.double() - want).abs() <= bound).all())
+
+
 @pytest.mark.parametrize("gdtype", [torch.bfloat16, torch.float32])
 def test_weight_grad_strides_and_rows_behind(gdtype):
     B = _pkg()
