@@ -397,6 +397,7 @@ __global__ void __launch_bounds__(32 * S4_MAX_WARPS, 1)
             for (int i = 0; kb + i < kb1; ++i) block(base, i, kb + i);
           }
         }
+        fence_proxy_async_smem();   // the slot has been read: the next copy may write it
         __syncwarp();
         if (lane == 0 && ok) request(slot);
         if (++slot == slots) {
@@ -824,6 +825,9 @@ __global__ void __launch_bounds__(S4M_THREADS, 1)
             s4_unpack_row(w.w, rot01, rot23, s[1], s24[1], out[16 + 4 * j + 2], out[16 + 4 * j + 3]);
           }
         }
+        // The reads are over before the next copy: without the fence nothing makes them
+        // wait, and the epilogue's stores may be queued ahead of them.
+        fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&raw_empty[i]);
         const int stage = i % S4M_STAGES;

@@ -353,3 +353,27 @@ def test_a_new_handle_is_ready_for_any_stream():
     assert s.query()
     x = c.tokens(7, torch.float32)
     assert torch.equal(sae.encode_pre(x), c.sae.encode_pre(x))
+
+
+@pytest.mark.parametrize("d,F,group,T", [(1536, 49152, 64, 300), (256, 70000, 32, 256),
+                                         (1536, 49152, 32, 3), (1536, 49152, 64, 21)])
+def test_more_feature_tiles_than_sms(d, F, group, T):
+    """An SM goes on to further tiles while the last one's features are being stored:
+    every call gives the same bits, within the bound."""
+    B = _pkg()
+    gen = torch.Generator(device=DEV).manual_seed(d + F + T)
+    codes, scales = B.quantize4_rows(torch.randn(F, d, device=DEV, generator=gen) / d ** 0.5, group)
+    sae = B.B200SAE4.from_codes(codes, scales, torch.zeros(F, device=DEV), codes, scales,
+                                torch.zeros(d, device=DEV), torch.zeros(F, device=DEV), group=group)
+    x = torch.randn(T, d, device=DEV, generator=gen).bfloat16()
+    q = torch.stack((codes & 15, codes >> 4), 2).reshape(F, d).double() - 8
+    w = q * scales.double().repeat_interleave(group, 1)[:, :d]
+    want, size = x.double() @ w.t(), x.double().abs() @ w.abs().t()
+    del q, w
+    room = 2.0 ** -23 * (64 + d / 256) * size + 2.0 ** -23 * want.abs() + 1e-37
+    other = torch.empty(256 << 20, device=DEV, dtype=torch.uint8)
+    first = sae.encode_pre(x)
+    assert bool(((first.double() - want).abs() <= room).all())
+    for _ in range(5):
+        other.zero_()                    # the weights leave the L2 cache
+        assert torch.equal(sae.encode_pre(x), first)
