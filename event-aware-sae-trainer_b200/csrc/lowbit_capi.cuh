@@ -30,9 +30,11 @@ int check_act8(const void* codes, const void* steps, int64_t n_tokens, int64_t n
 constexpr int64_t kWgradPartBytes = int64_t(1) << 30;
 constexpr int64_t kWgradValueBytes = int64_t(128) << 20;
 // Tiles of 256 gradient columns from which expanding beforehand pays. 8192 tokens x
-// 1536 columns take (beforehand | by the kernel) 42 | 32 us for 256 gradient columns,
-// 60 | 58 for 1536, 73 | 79 for 2304, 118 | 142 for 4096. With three parts of g the
-// kernel's own expansion is hidden behind their products.
+// 1536 columns take (beforehand | by the kernel) 48 | 40 us for 256 gradient columns,
+// 67 | 65 for 1536, 77 | 80 for 2304, 122 | 133 for 4096. With three parts of g the
+// kernel's own expansion is hidden behind their products. (Where the codes of all
+// tokens exceed kWgradValueBytes this is not so: 4096 tokens x 49152 columns by 2304
+// take 2520 | 970 us, the output being read and written for each 1024 tokens.)
 constexpr int64_t kWgradExpandTiles = 7;
 struct Wgrad8Plan {
   int parts;              // 0: g itself

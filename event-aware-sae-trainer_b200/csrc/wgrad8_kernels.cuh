@@ -2,12 +2,13 @@
 //
 //   D[c, n] = sum_t v[t, c] g[t, n]     v: int8 codes x power-of-two steps, g: bf16
 //
-// on tcgen05 (cta_group::2). The contraction runs over the tokens, and both
+// on tcgen05. The contraction runs over the tokens, and both
 // operands are stored token by token, so both are used with their output
 // dimension contiguous ("MN-major") and nothing is transposed:
 //   * a pair of CTAs computes 256 checkpoint columns x 256 gradient columns;
-//     each CTA holds 128 of either for 64 tokens per stage (16 KiB + 16 KiB);
-//   * g comes by TMA, two boxes of 64 columns x 64 tokens with 128-byte swizzle;
+//     each CTA holds 128 of the former (16 KiB) for 64 tokens per stage, and 128
+//     of the latter (or all 256, see WgConfig::PAIRED);
+//   * g comes by TMA, in boxes of 64 columns x 64 tokens with 128-byte swizzle;
 //   * codes and steps come by TMA into a ring of their own (9 KiB a stage);
 //     twelve warps expand them to bf16 (exact: 7-bit codes, power-of-two
 //     steps) into the swizzled layout.
@@ -48,11 +49,22 @@ constexpr int WG_GROUP_WARPS = 4, WG_GROUPS = WG_EXPAND_WARPS / WG_GROUP_WARPS;
 // PARTS: bf16 parts of g (3 only with EXPAND).
 template <bool EXPAND, int PARTS>
 struct WgConfig {
-  static constexpr int STAGES = PARTS == 3 ? 3 : EXPAND ? 5 : 7;
-  static constexpr int RAW_STAGES = PARTS == 3 ? 3 : EXPAND ? 6 : 0;
+  // A pair multiplies together (cta_group::2), each CTA with half of g's tile. What
+  // the other CTA expands then has to be released to the leader at cluster scope,
+  // and each such arrival takes about 2200 cycles. Behind the products of three parts
+  // they are hidden (164 | 166 us for 4096 tokens x 16384 columns by 512 gradients, with
+  // arrivals of CTA scope, which order nothing for another CTA, and these). With one
+  // part they are not (4096 x 49152 by 1536: 590 | 890 us), so there each CTA
+  // multiplies for itself, with a whole tile of g: 640 us, and for 8192 x 1536 by 256,
+  // 768 and 1536 gradients 39, 47 and 62 as against 41, 49 and 63.
+  static constexpr bool PAIRED = !EXPAND || PARTS == 3;
+  static constexpr int G_BOXES = PAIRED ? 2 : 4;   // of 64 gradient columns, a part and CTA
+  static constexpr int STAGES = PARTS == 3 ? 3 : EXPAND ? 4 : 7;
+  static constexpr int RAW_STAGES = EXPAND ? 3 : 0;
   // Stages per tensor-core accumulation: 32 products of 16 tokens, or 24 of three parts.
   static constexpr int CHUNK = PARTS == 3 ? 2 : 8;
-  static constexpr int STAGE_BYTES = (1 + PARTS) * WG_OPERAND_BYTES;
+  static constexpr int G_BYTES = G_BOXES * WG_BOX_BYTES;
+  static constexpr int STAGE_BYTES = WG_OPERAND_BYTES + PARTS * G_BYTES;
   // warpgroups: TMA + MMA, 3 x expand, 2 x epilogue
   static constexpr int EPI_WARP0 = 4 + (EXPAND ? WG_EXPAND_WARPS : 0);
   static constexpr int THREADS = 32 * (EPI_WARP0 + 8);
@@ -100,13 +112,6 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.b32 %0, 1, 0, P;\n\t}"
                : "=r"(p));
   return p != 0;
-}
-
-// Arrive at the leader's barrier after writing this CTA's own shared memory for
-// the tensor cores. fence.proxy.async has put the data where the MMA reads it;
-// a cluster-scope release on top made each arrival take about 2400 cycles.
-__device__ __forceinline__ void wg_arrive_leader(uint32_t leader_bar) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(leader_bar) : "memory");
 }
 
 // Descriptor of an MN-major bf16 tile in 128-byte swizzle: boxes of 64 columns
@@ -215,17 +220,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WgConfig<EXPAND, PAR
                   const __grid_constant__ Wgrad8Args a) {
   using Cfg = WgConfig<EXPAND, PARTS>;
   constexpr int STAGES = Cfg::STAGES, RAW_STAGES = Cfg::RAW_STAGES, CHUNK = Cfg::CHUNK;
-  constexpr int B_BYTES = PARTS * WG_OPERAND_BYTES;
+  constexpr bool PAIRED = Cfg::PAIRED;
+  constexpr int G_BYTES = Cfg::G_BYTES, B_BYTES = PARTS * G_BYTES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);   // still known to be shared memory
   uint8_t* s_a = smem;                                   // expanded codes
   uint8_t* s_b = smem + STAGES * WG_OPERAND_BYTES;       // g
   uint8_t* s_raw = smem + STAGES * Cfg::STAGE_BYTES;     // codes and steps as stored
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_raw + RAW_STAGES * WG_RAW_BYTES);
-  uint64_t* full = bars;                       // leader: both CTAs' copies and expanding warps
+  uint64_t* full = bars;                       // copies and expanding warps (PAIRED: both CTAs', at the leader)
   uint64_t* empty = bars + STAGES;          // each CTA: stage free
   uint64_t* acc_full = bars + 2 * STAGES;   // each CTA
-  uint64_t* acc_empty = bars + 2 * STAGES + 2;   // leader: 16 epilogue warps
+  uint64_t* acc_empty = bars + 2 * STAGES + 2;   // epilogue warps (PAIRED: both CTAs', at the leader)
   uint64_t* drain = bars + 2 * STAGES + 4;
   uint64_t* done_bar = bars + 2 * STAGES + 5;
   uint64_t* raw_full = bars + 2 * STAGES + 6;    // each CTA: its own copies
@@ -239,12 +245,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WgConfig<EXPAND, PAR
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full[s], EXPAND ? 1 + 2 * WG_GROUP_WARPS : 1);
+      mbar_init(&full[s], EXPAND ? 1 + (PAIRED ? 2 : 1) * WG_GROUP_WARPS : 1);
       mbar_init(&empty[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], 16);
+      mbar_init(&acc_empty[i], PAIRED ? 16 : 8);
     }
     for (int s = 0; s < RAW_STAGES; ++s) {
       mbar_init(&raw_full[s], 1);
@@ -256,8 +262,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WgConfig<EXPAND, PAR
     fence_barrier_init();
   }
   if (warp == 1) {
-    tmem_alloc_pair(tmem_holder, TC_TMEM_COLS);
-    tmem_relinquish_pair();
+    if constexpr (PAIRED) {
+      tmem_alloc_pair(tmem_holder, TC_TMEM_COLS);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_holder, TC_TMEM_COLS);
+      tmem_relinquish();
+    }
   }
   if (warp == 0 && lane == 0) {
     prefetch_tmap(&tm_g);
@@ -266,7 +277,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WgConfig<EXPAND, PAR
   }
   tc_fence_before();
   __syncthreads();
-  cluster_sync_all();
+  if constexpr (PAIRED) cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
   const int pairs = gridDim.x >> 1;
@@ -282,7 +293,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WgConfig<EXPAND, PAR
       const uint32_t lbar = mapa_shared(smem_u32(full), 0);
       for (int u = pair; u < total && ok; u += pairs) {
         const Wgrad8Unit w = wgrad8_unit(a, u);
-        const int n0 = w.n * 256 + static_cast<int>(rank) * 128;
+        const int n0 = w.n * 256 + (PAIRED ? static_cast<int>(rank) * 128 : 0);
         const int c0 = w.m * 256 + static_cast<int>(rank) * 128;
         for (int kb = w.kb0; kb < w.kb1; ++kb, st.next()) {
           if (!wg_wait(&empty[st.s], st.ph ^ 1, abort_flag)) {
@@ -290,7 +301,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WgConfig<EXPAND, PAR
             break;
           }
           uint8_t* dst = s_b + st.s * B_BYTES;
-          if (leader) mbar_arrive_expect_tx(&full[st.s], 2 * (EXPAND ? B_BYTES : Cfg::STAGE_BYTES));
+          if (leader || !PAIRED)
+            mbar_arrive_expect_tx(&full[st.s], (PAIRED ? 2 : 1) * (EXPAND ? B_BYTES : Cfg::STAGE_BYTES));
           if constexpr (!EXPAND) {
             uint8_t* da = s_a + st.s * WG_OPERAND_BYTES;
             tma_load_2d_pair(da, &tm_codes, lbar + 8 * st.s, c0, kb * WG_TOK);
@@ -299,9 +311,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WgConfig<EXPAND, PAR
 #pragma unroll
           for (int i = 0; i < PARTS; ++i) {
             const int row = i * a.part_rows + kb * WG_TOK;
-            uint8_t* db = dst + i * WG_OPERAND_BYTES;
-            tma_load_2d_pair(db, &tm_g, lbar + 8 * st.s, n0, row);
-            tma_load_2d_pair(db + WG_BOX_BYTES, &tm_g, lbar + 8 * st.s, n0 + 64, row);
+#pragma unroll
+            for (int b = 0; b < Cfg::G_BOXES; ++b) {
+              uint8_t* db = dst + i * G_BYTES + b * WG_BOX_BYTES;
+              if constexpr (PAIRED)
+                tma_load_2d_pair(db, &tm_g, lbar + 8 * st.s, n0 + 64 * b, row);
+              else
+                tma_load_2d(db, &tm_g, &full[st.s], n0 + 64 * b, row);
+            }
           }
         }
       }
@@ -335,17 +352,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WgConfig<EXPAND, PAR
         while (globaltimer_ns() - t0 < 1000000ull) {
         }
       }
-    } else if (warp == 1 && leader) {
+    } else if (warp == 1 && (leader || !PAIRED)) {
       // ------------------------------------------------------- MMA issue
-      constexpr uint32_t idesc = idesc_bf16_f32(256, 256) | kIdescMnMajor;
+      constexpr uint32_t idesc = idesc_bf16_f32(PAIRED ? 256 : 128, 256) | kIdescMnMajor;
       const uint64_t ad0 = smem_desc_mn_sw128(s_a), bd0 = smem_desc_mn_sw128(s_b);
+      // what the other CTA's threads have written is read by the products as well
+      auto wait_all = [&](uint64_t* bar, uint32_t parity) {
+        return PAIRED ? wg_wait_cluster(bar, parity, abort_flag) : wg_wait(bar, parity, abort_flag);
+      };
+      auto commit = [](uint64_t* bar) {
+        if constexpr (PAIRED) tc_commit_pair_both(bar);
+        else tc_commit(bar);
+      };
       Ring<STAGES> st;
       Ring<2> acc;
       bool ok = true, any = false;
       for (int u = pair; u < total && ok; u += pairs) {
         const Wgrad8Unit w = wgrad8_unit(a, u);
         for (int left = w.kb1 - w.kb0; left > 0 && ok; left -= CHUNK, acc.next()) {
-          if (!__all_sync(0xffffffffu, wg_wait_cluster(&acc_empty[acc.s], acc.ph ^ 1, abort_flag))) {
+          if (!__all_sync(0xffffffffu, wait_all(&acc_empty[acc.s], acc.ph ^ 1))) {
             ok = false;
             break;
           }
@@ -353,7 +378,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WgConfig<EXPAND, PAR
           const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc.s * 256);
           uint32_t add = 0;
           for (int k = min(left, CHUNK); k > 0; --k, st.next()) {
-            if (!__all_sync(0xffffffffu, wg_wait(&full[st.s], st.ph, abort_flag))) {
+            if (!__all_sync(0xffffffffu, wait_all(&full[st.s], st.ph))) {
               ok = false;
               break;
             }
@@ -362,24 +387,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WgConfig<EXPAND, PAR
             const uint64_t bd = bd0 + static_cast<uint32_t>(st.s * (B_BYTES >> 4));
             if (elect_one()) {
 #pragma unroll
-              for (int i = 0; i < PARTS; ++i)
+              for (int i = 0; i < PARTS; ++i) {
 #pragma unroll
-                for (int kk = 0; kk < WG_TOK / 16; ++kk)
+                for (int kk = 0; kk < WG_TOK / 16; ++kk) {
                   // 16 tokens further: two groups of 8 rows, 2048 bytes
-                  tc_mma_bf16_pair(d_tmem, ad + 128 * kk, bd + i * (WG_OPERAND_BYTES >> 4) + 128 * kk,
-                                   idesc, i + kk > 0 ? 1u : add);
-              tc_commit_pair_both(&empty[st.s]);
+                  const uint64_t bk = bd + i * (G_BYTES >> 4) + 128 * kk;
+                  if constexpr (PAIRED)
+                    tc_mma_bf16_pair(d_tmem, ad + 128 * kk, bk, idesc, i + kk > 0 ? 1u : add);
+                  else
+                    tc_mma_bf16(d_tmem, ad + 128 * kk, bk, idesc, i + kk > 0 ? 1u : add);
+                }
+              }
+              commit(&empty[st.s]);
             }
             __syncwarp();
             add = 1;
             any = true;
           }
-          if (ok && elect_one()) tc_commit_pair_both(&acc_full[acc.s]);
+          if (ok && elect_one()) commit(&acc_full[acc.s]);
           __syncwarp();
         }
       }
       if (!ok && any) {
-        if (elect_one()) tc_commit_pair_local(drain);
+        if (elect_one()) {
+          if constexpr (PAIRED) tc_commit_pair_local(drain);
+          else tc_commit(drain);
+        }
         __syncwarp();
         mbar_wait(drain, 0, nullptr);
       }
@@ -450,7 +483,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WgConfig<EXPAND, PAR
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) wg_arrive_leader(lbar + 8 * st.s);
+        if (lane == 0) {
+          if constexpr (PAIRED) mbar_arrive_remote(lbar + 8 * st.s);
+          else mbar_arrive(&full[st.s]);
+        }
       }
     }
   } else {
@@ -482,7 +518,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WgConfig<EXPAND, PAR
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_remote(acc.s ? leader_empty1 : leader_empty0);
+        if (lane == 0) {
+          if constexpr (PAIRED) mbar_arrive_remote(acc.s ? leader_empty1 : leader_empty0);
+          else mbar_arrive(&acc_empty[acc.s]);
+        }
       }
       if (!ok) break;
       const int64_t c = static_cast<int64_t>(w.m) * 256 + rank * 128 + q * 32 + lane;
@@ -523,13 +562,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WgConfig<EXPAND, PAR
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
-    if (lane == 0) {
-      mbar_arrive_remote(mapa_shared(smem_u32(done_bar), rank ^ 1u));
-      mbar_wait_cluster(done_bar, 0, nullptr);
+    if constexpr (PAIRED) {
+      if (lane == 0) {
+        mbar_arrive_remote(mapa_shared(smem_u32(done_bar), rank ^ 1u));
+        mbar_wait_cluster(done_bar, 0, nullptr);
+      }
+      __syncwarp();
+      tc_fence_after();
+      tmem_dealloc_pair(tmem_base, TC_TMEM_COLS);
+    } else {
+      tc_fence_after();
+      tmem_dealloc(tmem_base, TC_TMEM_COLS);
     }
-    __syncwarp();
-    tc_fence_after();
-    tmem_dealloc_pair(tmem_base, TC_TMEM_COLS);
   }
 }
 
