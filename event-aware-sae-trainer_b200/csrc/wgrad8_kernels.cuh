@@ -128,18 +128,19 @@ __device__ __forceinline__ uint64_t smem_desc_mn_sw128(const void* tile) {
 }
 constexpr uint32_t kIdescMnMajor = (1u << 15) | (1u << 16);   // A and B are MN-major
 
-// 32 lanes x 16 consecutive fp32 columns.
+// 32 lanes x 16 consecutive fp32 columns. Load and wait are one statement: between
+// two, nothing would keep a use of the registers behind the wait.
 __device__ __forceinline__ void tmem_ld_16cols(uint32_t taddr, float (&v)[16]) {
   uint32_t r[16];
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
         "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
         "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr)
       : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
