@@ -211,7 +211,8 @@ int launch_after(const char* what, void (*kernel)(Params...), dim3 grid, int thr
   return check_launch(what);
 }
 
-constexpr size_t kS4Smem = 224 * 1024;
+constexpr size_t kS4Smem = 224 * 1024, kS4LimbBytes = 160 * 1024;   // the latter at most
+static_assert(8 * s4_limb_pitch(SAE4_MAX_D_IN / S4_COLS) <= kS4LimbBytes, "one pair of tokens fits");
 size_t s4_limb_bytes(const S4Encoder& e, int nt) {
   return static_cast<size_t>(8) * nt * s4_limb_pitch(e.kblocks);
 }
@@ -228,19 +229,25 @@ int s4_encode_launch(const S4Encoder& e, const void* x, int64_t ldx, int n_tok, 
                          static_cast<int>(kS4Smem));
   });
   // Warps per block: the SM's tiles in even rounds. Split a tile's columns
-  // while that gives warps the SM has room for.
+  // while that gives warps the SM has room for, and each a slot of its ring.
   constexpr int max_warps = S4_MAX_WARPS;
   const int sms = std::max(1, device_info().sm_count);
   const int64_t per_sm = (s4_tiles(e.F) + sms - 1) / sms;
   const int64_t rounds = (per_sm + max_warps - 1) / max_warps;
   const int at_once = static_cast<int>((per_sm + rounds - 1) / rounds);
+  auto fixed_bytes = [&](int split) {   // limbs, and the sums to be joined
+    return s4_limb_bytes(e, NT) + (split > 1 ? static_cast<size_t>(at_once) * split * NT * 512 : 0);
+  };
+  auto slot_bytes = [&](int split) { return static_cast<size_t>(at_once) * split * s4_slot_bytes(SPB); };
   int ks = 1;
-  while (2 * ks * at_once <= max_warps && 2 * ks <= s4_kchunks(e.kblocks)) ks *= 2;
+  while (2 * ks * at_once <= max_warps && 2 * ks <= s4_kchunks(e.kblocks) &&
+         fixed_bytes(2 * ks) + slot_bytes(2 * ks) <= kS4Smem)
+    ks *= 2;
   const int warps = at_once * ks;
-  const size_t fixed = s4_limb_bytes(e, NT) + (ks > 1 ? static_cast<size_t>(warps) * NT * 512 : 0);
-  const size_t per_slot = static_cast<size_t>(warps) * s4_slot_bytes(SPB);
+  const size_t fixed = fixed_bytes(ks), per_slot = slot_bytes(ks);
+  static_assert(kS4LimbBytes + S4_MAX_WARPS * s4_slot_bytes(SPB) <= kS4Smem,
+                "a tile that is not split has room for a slot a warp");
   const int slots = static_cast<int>(std::min<size_t>(S4_MAX_SLOTS, (kS4Smem - fixed) / per_slot));
-  if (slots < 1) return fail(SAE_ERR_UNSUPPORTED_SHAPE, "sae4_encode: d_in too large");
   const int grid = static_cast<int>(std::min<int64_t>(sms, s4_tiles(e.F)));
   const int vec = vec_rows(x, ldx, sizeof(XT) == 4 ? SAE_DTYPE_F32 : SAE_DTYPE_BF16);
   s4_encode_few_kernel<NT, SPB, XT><<<grid, warps * 32, fixed + slots * per_slot, stream>>>(
@@ -253,7 +260,7 @@ int s4_encode_tokens(const S4Encoder& e, const void* x, int64_t ldx, int64_t n_t
                      const S4Out& o, cudaStream_t stream) {
   for (int64_t t0 = 0; t0 < n_tokens;) {
     // two tokens' limbs at a time where four tokens' leave the weights no room
-    const int nt = n_tokens - t0 > 2 && s4_limb_bytes(e, 2) <= 160 * 1024 ? 2 : 1;
+    const int nt = n_tokens - t0 > 2 && s4_limb_bytes(e, 2) <= kS4LimbBytes ? 2 : 1;
     const int n_tok = static_cast<int>(std::min<int64_t>(2 * nt, n_tokens - t0));
     S4Out part = o;
     part.out += t0 * o.ldo;

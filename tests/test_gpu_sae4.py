@@ -377,3 +377,40 @@ def test_more_feature_tiles_than_sms(d, F, group, T):
     for _ in range(5):
         other.zero_()                    # the weights leave the L2 cache
         assert torch.equal(sae.encode_pre(x), first)
+
+
+@pytest.mark.parametrize("T", [3, 4, 1027])
+@pytest.mark.parametrize("d,F,group", [(9300, 6000, 32), (10000, 28000, 64), (10176, 25000, 128)])
+def test_wide_inputs_of_three_and_four_tokens(d, F, group, T):
+    """Widths at which four tokens, all of an SM's warps and their buffers do not fit
+    together: fewer warps share a tile then. reconstruct of 1027 tokens ends with three."""
+    B = _pkg()
+    gen = torch.Generator(device=DEV).manual_seed(d + F)
+    rows = lambda: B.quantize4_rows(torch.randn(F, d, device=DEV, generator=gen) / d ** 0.5, group)  # noqa: E731
+    enc, dec = rows(), rows()
+    b_enc = torch.randn(F, device=DEV, generator=gen)
+    b_dec = torch.randn(d, device=DEV, generator=gen)
+    sae = B.B200SAE4.from_codes(*enc, b_enc, *dec, b_dec, torch.full((F,), np.log(3.0), device=DEV),
+                                group=group)
+    x = torch.randn(T, d, device=DEV, generator=gen).bfloat16()
+    x_hat, counts = sae.reconstruct(x)
+    x, x_hat, counts = x[-3:], x_hat[-3:], counts[-3:]
+    pre, feat = sae.encode_pre(x), sae.encode(x)
+    assert torch.equal(feat, torch.where(pre > sae._theta, pre, 0.0))
+
+    def weights(codes, scales):
+        q = torch.stack((codes & 15, codes >> 4), 2).reshape(F, d).double() - 8
+        return q * scales.double().repeat_interleave(group, 1)[:, :d]
+
+    xc = (x.float() - b_dec).bfloat16().double()
+    w = weights(*enc)
+    want = xc @ w.t() + b_enc.double()
+    room = 2.0 ** -23 * (64 + d / 256) * (xc.abs() @ w.abs().t()) + 2.0 ** -23 * (
+        b_enc.double().abs() + want.abs()) + 1e-37
+    assert bool(((pre.double() - want).abs() <= room).all())
+    assert torch.equal(counts, (feat != 0).sum(1, dtype=torch.int32))
+    w = weights(*dec)
+    want = feat.double() @ w + b_dec.double()
+    room = 2.0 ** -24 * (counts[:, None] + 4) * (feat.double().abs() @ w.abs()) \
+        + 2.0 ** -23 * want.abs() + 1e-37
+    assert bool(((x_hat.double() - want).abs() <= room).all())
