@@ -160,13 +160,14 @@ class _EncoderPre(torch.autograd.Function):
             w_used = weight.detach()
         L.call("sae_b200_encode_pre", model, L.ptr(x), _dt_code(x), B, L.ptr(pre), _dt_code(pre),
                L.ptr(xc), 0, None, 0, _stream())
-        ctx.keep8 = keep8 and any(ctx.needs_input_grad)   # else no backward reads it
-        if ctx.keep8:
+        if not ctx.needs_input_grad[1]:      # xc is read for the weight's gradient alone
+            ctx.save_for_backward(w_used)
+        elif keep8:
             held = checkpoint8(xc)
-            ctx.save_for_backward(held.codes, held.step_rows, w_used)
-            ctx.xc_dtype = xc.dtype
+            ctx.save_for_backward(w_used, held.codes, held.step_rows)
         else:
-            ctx.save_for_backward(xc, w_used)
+            ctx.save_for_backward(w_used, xc)
+        ctx.xc_dtype = xc.dtype
         ctx.param_dtypes = (weight.dtype, b_enc.dtype, b_dec.dtype)
         return pre
 
@@ -175,15 +176,14 @@ class _EncoderPre(torch.autograd.Function):
         dpre = dpre.contiguous()
         B, F = dpre.shape
         dev = dpre.device
-        if ctx.keep8:
-            codes, steps, w = ctx.saved_tensors
-            d = w.shape[1]
-            dW = Act8(codes, steps, (B, d), ctx.xc_dtype).weight_grad(dpre)
-        else:
-            xc, w = ctx.saved_tensors
-            d = xc.shape[1]
+        w, *kept = ctx.saved_tensors
+        d = w.shape[1]
+        dW = None                                                       # dpre^T xc
+        if len(kept) == 2:
+            dW = Act8(*kept, (B, d), ctx.xc_dtype).weight_grad(dpre)
+        elif kept:
             dW = torch.empty(F, d, device=dev, dtype=torch.float32)
-            gemm(F, d, B, dpre, 1, F, xc, 1, d, dW, d, 1)              # dpre^T xc
+            gemm(F, d, B, dpre, 1, F, kept[0], 1, d, dW, d, 1)
         db_enc = torch.empty(F, device=dev, dtype=torch.float32)
         column_sum(dpre, db_enc)                                        # sum_b dpre
         db_dec = torch.empty(1, d, device=dev, dtype=torch.float32)
@@ -252,22 +252,20 @@ class _Decode(torch.autograd.Function):
             a_in, w_in = acts, fm.detach()
             out = torch.empty(B, d, device=acts.device, dtype=torch.float32)
             gemm(B, d, F, a_in, F, 1, w_in, 1, d, out, d, 1, bias=b_dec.detach())
-        ctx.keep8 = keep8 and any(ctx.needs_input_grad)
-        if ctx.keep8:
+        if not ctx.needs_input_grad[1]:      # acts are read for the weight's gradient alone
+            ctx.save_for_backward(w_in)
+        elif keep8:
             held = checkpoint8(a_in)
-            ctx.save_for_backward(held.codes, held.step_rows, w_in)
-            ctx.a_dtype = a_in.dtype
+            ctx.save_for_backward(w_in, held.codes, held.step_rows)
         else:
-            ctx.save_for_backward(a_in, w_in)
+            ctx.save_for_backward(w_in, a_in)
+        ctx.a_dtype = a_in.dtype
         ctx.bf = bf
         return out
 
     @staticmethod
     def backward(ctx, go):
-        if ctx.keep8:
-            codes, steps, w_in = ctx.saved_tensors
-        else:
-            a_in, w_in = ctx.saved_tensors
+        w_in, *kept = ctx.saved_tensors
         go = go.contiguous().float()
         B, d = go.shape
         F = w_in.shape[0]
@@ -278,13 +276,12 @@ class _Decode(torch.autograd.Function):
                              dtype=torch.bfloat16 if ctx.bf else torch.float32)
             gemm(B, F, d, g_in, d, 1, w_in, d, 1, ga, F, 1)             # go W_dec
             grad_acts = ga.float()
-        grad_w = None
-        if ctx.needs_input_grad[1]:
-            if ctx.keep8:                                               # acts^T go
-                g_fm = Act8(codes, steps, (B, F), ctx.a_dtype).weight_grad(g_in, transposed=True)
-            else:
-                g_fm = torch.empty(F, d, device=go.device, dtype=torch.float32)
-                gemm(F, d, B, a_in, 1, F, g_in, 1, d, g_fm, d, 1)
+        grad_w = None                                                   # acts^T go
+        if len(kept) == 2:
+            grad_w = Act8(*kept, (B, F), ctx.a_dtype).weight_grad(g_in, transposed=True).t()
+        elif kept:
+            g_fm = torch.empty(F, d, device=go.device, dtype=torch.float32)
+            gemm(F, d, B, kept[0], 1, F, g_in, 1, d, g_fm, d, 1)
             grad_w = g_fm.t()
         grad_b = None
         if ctx.needs_input_grad[2]:

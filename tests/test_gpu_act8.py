@@ -547,3 +547,37 @@ def test_module_checkpoint_memory_and_refusals():
     with torch.no_grad():
         b = sae(x)
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("bits", [None, 8])
+@pytest.mark.parametrize("frozen", ["W_enc.weight", "W_dec.weight"])
+def test_module_with_a_frozen_weight_keeps_nothing_for_it(frozen, bits):
+    """The encoder's input and the decoder's are kept for their weight gradients alone:
+    a frozen weight costs neither their bytes nor a product, and the other gradients
+    are the same bits."""
+    B = _pkg()
+    sae = B.make_sae(1024, 8192, seed=0).cuda()
+    sae.checkpoint_bits = bits
+    T = 1024
+    x = torch.randn(T, 1024, device=DEV)
+
+    def run():
+        for p in sae.parameters():
+            p.grad = None
+        torch.cuda.synchronize()
+        base = torch.cuda.memory_allocated()
+        with torch.autocast("cuda", torch.bfloat16):
+            x_hat, acts = sae(x)
+        kept = torch.cuda.memory_allocated() - base - acts.numel() * 4 - x_hat.numel() * 4
+        (x_hat.square().sum() + acts.sum()).backward()
+        return kept, {n: p.grad for n, p in sae.named_parameters()}
+
+    run()
+    whole, want = run()
+    dict(sae.named_parameters())[frozen].requires_grad_(False)
+    less, got = run()
+    assert got.pop(frozen) is None
+    for n, g in got.items():
+        assert torch.equal(g, want[n]), n
+    elements = T * (1024 if frozen == "W_enc.weight" else 8192)
+    assert whole - less >= elements * (1 if bits == 8 else 2)
