@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(32 * S4_MAX_WARPS, 1)
         }
       };
       for (int kb = kb0; kb < kb1; kb += S4_CHUNK) {
-        ok = ok && mbar_wait(&bar[slot], phase, nullptr);
+        ok = __all_sync(0xffffffffu, ok && mbar_wait(&bar[slot], phase, nullptr));
         const uint8_t* base = s_ring + slot * slot_bytes;
         if (ok) {
           if (kb + S4_CHUNK <= kb1) {
@@ -732,14 +732,14 @@ __global__ void __launch_bounds__(S4M_THREADS, 1)
       for (int u = blockIdx.x; u < total && ok; u += gridDim.x) {
         int blocks = e.kblocks;
         while (blocks > 0 && ok) {
-          if (!wg_wait(&acc_empty[acc.s], acc.ph ^ 1, abort_flag)) {
+          if (!wg_wait_warp(&acc_empty[acc.s], acc.ph ^ 1, abort_flag)) {
             ok = false;
             break;
           }
           tc_fence_after();
           const uint32_t d_tmem = tmem_base + S4M_ACC_COL + acc.s * S4M_TOKENS;
           for (int k = 0; k < S4M_SUM_STAGES && blocks > 0; ++k, blocks -= S4_CHUNK, st.next()) {
-            if (!wg_wait(&full[st.s], st.ph, abort_flag)) {
+            if (!wg_wait_warp(&full[st.s], st.ph, abort_flag)) {
               ok = false;
               break;
             }
@@ -800,7 +800,7 @@ __global__ void __launch_bounds__(S4M_THREADS, 1)
 #pragma unroll
       for (int i = 0; i < S4M_RAW_STAGES; ++i) {
         if (i >= left) break;
-        if (!wg_wait(&raw_full[i], ph, abort_flag)) {
+        if (!wg_wait_warp(&raw_full[i], ph, abort_flag)) {
           left = 0;
           break;
         }
@@ -831,7 +831,7 @@ __global__ void __launch_bounds__(S4M_THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&raw_empty[i]);
         const int stage = i % S4M_STAGES;
-        if (!wg_wait(&empty[stage], (i / S4M_STAGES & 1) ^ 1, abort_flag)) {
+        if (!wg_wait_warp(&empty[stage], (i / S4M_STAGES & 1) ^ 1, abort_flag)) {
           left = 0;
           break;
         }
@@ -857,7 +857,7 @@ __global__ void __launch_bounds__(S4M_THREADS, 1)
 #pragma unroll
       for (int i = 0; i < S4M_TOKENS / 2; ++i) sum[i] = 0.f;
       for (int left = kchunks; left > 0; left -= S4M_SUM_STAGES, acc.next()) {
-        if (!wg_wait(&acc_full[acc.s], acc.ph, abort_flag)) {
+        if (!wg_wait_warp(&acc_full[acc.s], acc.ph, abort_flag)) {
           ok = false;
           break;
         }
