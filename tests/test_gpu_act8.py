@@ -581,3 +581,81 @@ def test_module_with_a_frozen_weight_keeps_nothing_for_it(frozen, bits):
         assert torch.equal(g, want[n]), n
     elements = T * (1024 if frozen == "W_enc.weight" else 8192)
     assert whole - less >= elements * (1 if bits == 8 else 2)
+
+
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("N", [1800, 1801])        # gradients read in place, or copied first
+def test_weight_grad_of_codes_expanded_in_several_launches(N, transposed):
+    """Many gradient columns of a wide checkpoint: the codes are expanded beforehand, a
+    part of the tokens at a time, the last one shorter; later launches add to the first."""
+    import ctypes
+    B = _pkg()
+    from sae_b200 import _lib as L
+    T, D = 3700, 33000
+    gen = torch.Generator(device=DEV).manual_seed(N)
+    x = torch.randn(T, D, device=DEV, generator=gen).bfloat16()
+    g = (torch.randn(T, N, device=DEV, generator=gen) * 1e-3).bfloat16()
+    a = B.checkpoint8(x)
+    need = ctypes.c_size_t(0)
+    L.call("sae_b200_weight_grad8_workspace_bytes", T, D, g.data_ptr(), L.DTYPE_BF16, N, N,
+           ctypes.byref(need))
+    values = need.value - (0 if N % 8 == 0 else 2 * 1808 * (need.value // (2 * (1808 + 33024))))
+    held = values // (2 * 33024)                     # tokens expanded at a time
+    assert T / 4 < held < T / 2 and T % held != 0
+    v, g64 = a.dequantize(torch.float32).double(), g.double()
+    want = g64.t() @ v
+    bound = 2.0 ** -23 * (64 + T / 256) * (g64.abs().t() @ v.abs())
+    del v, g64
+    base = torch.randn((D, N) if transposed else (N, D), device=DEV, generator=gen) * 1e-2
+    got = a.weight_grad(g, transposed=transposed)
+    acc = a.weight_grad(g, transposed=transposed, out=base.clone(), accumulate=True)
+    turn = (lambda t: t.t()) if transposed else (lambda t: t)
+    # each launch after the first rounds its sum with what is there
+    room = bound + 2 * 2.0 ** -24 * (want.abs() + bound) + 1e-37
+    assert bool(((turn(got).double() - want).abs() <= room).all())
+    room = bound + 3 * 2.0 ** -24 * (want.abs() + bound + turn(base).double().abs()) + 1e-37
+    assert bool(((turn(acc).double() - turn(base).double() - want).abs() <= room).all())
+    assert torch.equal(a.weight_grad(g, transposed=transposed), got)
+
+
+@pytest.mark.parametrize("base,unit", [(1.0, 2.0 ** -7), (1.0, 2.0 ** -15), (1.0, 2.0 ** -23),
+                                       (1.0 + 2.0 ** -8, 2.0 ** -23)])
+def test_weight_grad_uses_all_bits_of_fp32_gradients(base, unit):
+    """Tokens in pairs whose gradients base + k unit and -base leave sum k unit v, over one
+    stage of 64 tokens, in which the upper parts are added first, then the middle ones.
+
+    Units of 2^-7 and 2^-15: products have 15 bits, and what the upper parts leave is at
+    most 2^-8 sum |v| < 16, so every partial sum has 20 bits and is exact. base
+    1 + 2^-8, k >= 0: the upper parts 1 and the middle ones 2^-8 cancel, the lower ones are
+    k unit; exact. base 1, unit 2^-23: for k < 0 the upper part is 1 - 2^-8, so 2^-8 sum |v|
+    is left until the lower parts are added, and each of their eight products of 16
+    tokens may lose two units in the last place of that."""
+    B = _pkg()
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    v = torch.randint(-127, 128, (32, 160), device=DEV, generator=gen)
+    v[:, ::32] = 127                                  # the step of every group is 1
+    k = torch.randint(-100, 101, (32, 300), device=DEV, generator=gen)
+    room = torch.zeros(160, device=DEV, dtype=torch.float64)
+    if base != 1:
+        k = k.abs()
+    elif unit == 2.0 ** -23:
+        room = 8 * 2 * 2.0 ** -23 * 2.0 ** -8 * v.abs().sum(0).double()
+    x = v.repeat_interleave(2, 0).float()
+    g = torch.empty(64, 300, device=DEV)
+    g[0::2], g[1::2] = base + k * unit, -base
+    assert torch.equal(g[0::2].double() - base, k * unit)       # held by fp32
+    want = (k.t().double() @ v.double()) * unit
+    for transposed in (False, True):
+        got = B.checkpoint8(x).weight_grad(g, transposed=transposed)
+        off = ((got.t() if transposed else got).double() - want).abs()
+        assert bool((off <= room).all())
+
+
+def test_no_wait_ran_out():
+    """Kernels' waits are bounded; one that ran out, here or in a test before, is recorded."""
+    B = _pkg()
+    from sae_b200 import _lib as L
+    x = torch.randn(500, 640, device=DEV)
+    for g in (torch.randn(500, 700, device=DEV), torch.randn(500, 2000, device=DEV).bfloat16()):
+        B.checkpoint8(x).weight_grad(g)
+    assert L.device_status() == 0

@@ -414,3 +414,12 @@ def test_wide_inputs_of_three_and_four_tokens(d, F, group, T):
     room = 2.0 ** -24 * (counts[:, None] + 4) * (feat.double().abs() @ w.abs()) \
         + 2.0 ** -23 * want.abs() + 1e-37
     assert bool(((x_hat.double() - want).abs() <= room).all())
+
+
+def test_no_wait_ran_out():
+    """Kernels' waits are bounded; one that ran out, here or in a test before, is recorded."""
+    from sae_b200 import _lib as L
+    c = Case(512, 4096, 64)
+    for T in (1, 4, 40):
+        c.sae.reconstruct(c.tokens(T, torch.bfloat16))
+    assert L.device_status() == 0
