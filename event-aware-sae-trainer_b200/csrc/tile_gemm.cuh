@@ -341,6 +341,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
         if (c % (TILE_N / 2) == TILE_N / 2 - 32) e.end_half(c / (TILE_N / 2));
       }
       if (AUX == AUX_LOAD) {
+        fence_proxy_async_smem();   // the buffer has been read before TMA fills it again
         __syncwarp();
         if (lane == 0) mbar_arrive(aux_empty);
       }
@@ -704,6 +705,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC2_THREADS, 1)
       }
       e.end_half(h);
       if (AUX == AUX_LOAD) {
+        fence_proxy_async_smem();   // the buffer has been read before TMA fills it again
         __syncwarp();
         if (lane == 0) mbar_arrive(aux_empty);
       }
