@@ -273,9 +273,9 @@ int s4_encode_tokens(const S4Encoder& e, const void* x, int64_t ldx, int64_t n_t
   return SAE_OK;
 }
 
-// Tokens from which the tcgen05 kernel is the faster one. At 1536 x 49152 it takes
-// 23 us for 5 to 16 tokens (with the centring), the integer kernel 14 for one, 18 for
-// four and as much again for each further four; at 256 x 8192 8.5 against 5 and 6.
+// Tokens from which the tcgen05 kernel is the faster one. At 1536 x 49152, weights not
+// in L2, it takes 22 us for 5 to 16 tokens and 4 for the centring, the integer kernel 14
+// for one, 18 for four and as much again for each further four.
 constexpr int64_t kS4ManyTokens = 5;
 
 template <int SPB, int MODE>

@@ -174,8 +174,9 @@ __device__ __forceinline__ float s4_gate(float pre, float theta) {
 // (w << 4) & 0xf0f0f0f0 are eight bytes 16 q. So a token's xc is written as a
 // fixed-point number: with 2^E above its largest |xc|, rint(xc 2^(30 - E)) in
 // four signed bytes ("limbs"), each a column of the m16n8k32 s8 product. That
-// keeps every bit of an xc above 2^-23 of the largest and is off by 2^-31 of
-// the largest below (bf16 itself has 8 bits); the products and the sums over a
+// keeps every bit of an xc of at least 2^(E - 23), which 2^-22 of the largest always
+// is, and is off by at most 2^(E - 31), 2^-30 of the largest, below (bf16 itself has
+// 8 bits); the products and the sums over a
 // block of 64 columns are whole numbers below 2^21, exact. The integer
 // accumulator starts at the bits of 1.5 * 2^23, so it ends as the bits of
 // 1.5 * 2^23 + 16 S: a subtraction and one fma with the group's scale add it
@@ -188,7 +189,8 @@ __device__ __forceinline__ float s4_gate(float pre, float theta) {
 // warp order. Each warp streams its blocks through a ring of its own in shared
 // memory by bulk copies, a chunk (256 columns) a slot; they run on from
 // one tile into the next, so that the copies in flight, not the registers,
-// set the bandwidth. One token: 1536 x 49152 10 us, 4096 x 131072 50 us (5.5 TB/s).
+// set the bandwidth. One token, weights not in L2: 1536 x 49152 14 us
+// (2.8 TB/s), 4096 x 131072 50 us (5.7 TB/s).
 constexpr int S4_MAX_WARPS = 24;
 constexpr int S4_MAX_SLOTS = 8;
 
@@ -484,12 +486,12 @@ __global__ void __launch_bounds__(32 * S4_MAX_WARPS, 1)
 // As in the weight gradients, the tensor core's sums are closed every 512
 // columns and added in fp32 registers by eight epilogue warps, from two
 // accumulators in turn; the register file is divided with setmaxnreg.
-// 128 tokens at 2304 x 65536 take 47 us, 300 at 1536 x 49152 53 us (tensor cores 45%
-// busy, the integer pipe 48%). No one thing bounds it: with all of it in L2 the
-// former take 40 us, 37 without the unpacking arithmetic, 35 without the products, 35
-// without the stores and 24 without all three, which is the streaming of the weights
-// and, to every CTA anew, of the tokens. For 16 tokens the arithmetic bounds it: 31
-// us, and 23 without.
+// Weights not in L2, 128 tokens at 2304 x 65536 take 50 us, 300 at 1536 x 49152 56
+// (tensor cores 45 and 51% busy, the integer pipe 53 and 64%). No one thing bounds it:
+// with all of it in L2 the former took 40 us, 37 without the unpacking arithmetic, 35
+// without the products, 35 without the stores and 24 without all three, which is the
+// streaming of the weights and, to every CTA anew, of the tokens. 16 and 21 tokens at
+// 1536 x 49152 take 22 us, with the integer pipe 53% busy.
 constexpr int S4M_FEATURES = 128, S4M_TOKENS = 128;
 // A stage is a chunk, four column blocks. (Stages of one block and finer token rings
 // made no difference.)
@@ -793,7 +795,7 @@ __global__ void __launch_bounds__(S4M_THREADS, 1)
     for (int j = 0; j < 4; ++j) unit[j] = 16 * s4_unit(r & 7, j);
     const uint8_t* scale0 = s_raw + at + 512 + (r & 7) * 4;
     // A round of the raw ring at a time, so that slots and parities are constants
-    // (rings stepped at run time: 5 us more of the 53 for 300 tokens).
+    // (rings stepped at run time: 5 us more for 300 tokens).
     uint32_t ph = 0;
 #pragma unroll 1
     for (int left = units * kchunks; left > 0; left -= S4M_RAW_STAGES, ph ^= 1) {

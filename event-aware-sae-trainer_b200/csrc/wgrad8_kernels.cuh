@@ -27,9 +27,10 @@
 //
 // fp32 gradients are split into three bf16 parts (8 + 8 + 8 bits, exactly g). A
 // stage then holds all three, so that codes are expanded once for three products:
-// 4096 tokens x 8192 columns x 256 fp32 gradients take 49 us, 61 part after part.
+// 4096 tokens x 8192 columns x 256 fp32 gradients take 51 us, 61 part after part.
 // Bound by the tensor cores: 32768 tokens x 1536 columns x 49152 bf16 gradients take
-// 2.8 to 3.2 ms with the power the chip has (0.9 of a library product's burst rate).
+// 2.8 to 3.1 ms after a pause, and 3.3 call after call under the power limit (the library's
+// bf16 product of that size 3.2).
 #pragma once
 #include <cuda_bf16.h>
 #include <cstdint>

@@ -132,7 +132,7 @@ class Act8:
         """``sum_t g[t, n] v[t, c]`` over the tokens, v the checkpoint's values:
         float32 ``[N, D]``, or ``[D, N]`` when ``transposed``. ``g``: ``[..., N]``
         float32 or bfloat16 with the checkpoint's leading dimensions. ``out`` is
-        written, or added to when ``accumulate``."""
+        written, or added to when ``accumulate``. No gradient is recorded."""
         _cuda_float("g", g)
         if g.dim() != len(self.shape) or g.shape[:-1] != self.shape[:-1]:
             raise ValueError(f"g must have the checkpoint's leading dimensions "
@@ -169,8 +169,8 @@ class Act8:
 
 def checkpoint8(x: torch.Tensor) -> Act8:
     """Hold ``x [..., D]`` (float32 or bfloat16) at 8 bits per element; see ``Act8``.
-    An element is off by at most half its group's step, and the step is below
-    max|x| / 63.5 of its 32 columns. A group with an infinity or a NaN reads
+    An element is off by at most half its group's step; the step is at most
+    max|x| / 63.75 of its 32 columns, or 2^-126. A group with an infinity or a NaN reads
     back as NaN."""
     _cuda_float("x", x)
     if x.dim() < 2 or x.shape[-1] == 0:

@@ -335,8 +335,8 @@ class B200JumpReLUSAE(nn.Module):
         """8: forward passes that record a graph keep the encoder's input, the
         pre-activations and the decoder's input in 8 bits for the backward
         (half the bytes under bf16 autocast, a quarter in fp32). None (the
-        default): the tensors themselves. An ``x`` that needs a gradient is
-        kept as it is. ``ste_bandwidth`` must not change between a forward in
+        default): the tensors themselves. A frozen weight's operand is not kept
+        at all. An ``x`` that needs a gradient is kept as it is. ``ste_bandwidth`` must not change between a forward in
         8 bits and its backward."""
         return self.__dict__.get("_checkpoint_bits")
 

@@ -35,8 +35,9 @@ def _check_shape(F: int, d: int, group: int) -> None:
 
 
 def quantize4_rows(W: torch.Tensor, group: int = 64) -> Tuple[torch.Tensor, torch.Tensor]:
-    """``W [F, d]`` float32 as 4-bit codes ``uint8 [F, d / 2]`` (byte i: column
-    2 i + 8 in the low half, column 2 i + 1 in the high one) and ``bfloat16
+    """``W [F, d]`` float32 as 4-bit codes ``uint8 [F, d / 2]`` (byte i: the
+    code of column 2 i in the low half, of column 2 i + 1 in the high one, each
+    as q + 8) and ``bfloat16
     [F, ceil(d / group)]`` scales: max|w| / 7 rounded up to 5 significant bits."""
     _cuda_float("W", W)
     if W.dim() != 2 or W.dtype != torch.float32:
